@@ -541,7 +541,8 @@ MOE_B200_API int moe_b200_residual_norm_forward(moe_b200_engine_t* engine, const
  * d_hidden, d_y, d_gate (fp32, an element gate's in y's type), d_post_w and
  * d_pre_w (fp32 [hidden], overwritten).  d_hidden may be d_hidden_out itself,
  * d_y may be y itself.  The workspace holds each block's sums over its
- * tokens; it is needed for d_post_w, d_pre_w and a channel gate's d_gate. */
+ * tokens; it is needed for d_post_w, d_pre_w and a channel gate's d_gate (0
+ * bytes for a config that the call refuses). */
 MOE_B200_API uint64_t moe_b200_residual_norm_workspace_bytes(const moe_b200_residual_norm_cfg_t* cfg);
 MOE_B200_API int moe_b200_residual_norm_backward(moe_b200_engine_t* engine, const moe_b200_residual_norm_cfg_t* cfg,
                            const void* d_hidden_out, const void* d_x, const void* hidden_out, const void* y,

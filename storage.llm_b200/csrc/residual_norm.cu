@@ -992,10 +992,11 @@ int moe_b200_residual_norm_forward(moe_b200_engine_t* eng, const moe_b200_residu
     return launched(NORM_BY_TYPE(CALL_NORM), "residual norm", err);
 }
 
-uint64_t moe_b200_residual_norm_workspace_bytes(const moe_b200_residual_norm_cfg_t* cfg) {
-    if (!cfg) return 0;
-    const uint64_t slots = cfg->gate == MOE_B200_GATE_CHANNEL ? 3 : 2;
-    return std::min<uint64_t>(cfg->tokens, norm_blocks(cfg->hidden)) * slots * cfg->hidden * 4;
+uint64_t moe_b200_residual_norm_workspace_bytes(const moe_b200_residual_norm_cfg_t* cfg_in) {
+    moe_b200_residual_norm_cfg_t cfg;
+    if (!check_norm(cfg_in, &cfg, nullptr)) return 0;  // the call itself says why
+    const uint64_t slots = cfg.gate == MOE_B200_GATE_CHANNEL ? 3 : 2;
+    return std::min<uint64_t>(cfg.tokens, norm_blocks(cfg.hidden)) * slots * cfg.hidden * 4;
 }
 
 int moe_b200_residual_norm_backward(moe_b200_engine_t* eng, const moe_b200_residual_norm_cfg_t* cfg_in,
