@@ -207,14 +207,41 @@ _TYPE_BYTES = {DTYPE_F32: 4, DTYPE_BF16: 2, DTYPE_F16: 2, DTYPE_E8M0: 1}
 _KIND = {}  # torch dtype -> DTYPE_*, filled as types are met (this module does not import torch)
 
 
-def _dev(dev: int, name: str, t, element_bytes: int, count: int) -> Optional[int]:
+class _Types(set):
+    """The element types an operand may have, by name; the set holds the torch
+    dtypes of these names that have been met (a lookup a call)."""
+
+    def __init__(self, *names: str):
+        super().__init__()
+        self.names = names
+
+
+_F32, _I32, _U32, _U8 = (_Types("torch.float32"), _Types("torch.int32"), _Types("torch.uint32", "torch.int32"),
+                         _Types("torch.uint8"))
+_CODES = {Q4_E2M1: _Types("torch.uint8", "torch.int8", "torch.float4_e2m1fn_x2"),
+          Q4_INT4: _Types("torch.uint8", "torch.int8")}
+_SCALES = {DTYPE_F32: _F32, DTYPE_BF16: _Types("torch.bfloat16"), DTYPE_F16: _Types("torch.float16"),
+           DTYPE_E8M0: _Types("torch.uint8", "torch.float8_e8m0fnu")}
+
+
+def _dev(dev: int, name: str, t, element_bytes: int, count: int, types: Optional[_Types] = None) -> Optional[int]:
     """The pointer of an operand of `count` values on device `dev`, after a
-    check that its memory holds them.  element_bytes 0: any bytes."""
+    check that its memory holds them and that they are of one of `types`
+    (None: any of that size).  element_bytes 0: any bytes."""
     if t is None:
         return None
     if t.get_device() != dev:
         raise MoEError(f"{name} is on {t.device}, the engine on cuda:{dev}")
-    if element_bytes and (t.itemsize != element_bytes or t.nbytes < count * element_bytes or not t.is_contiguous()):
+    if types is None:
+        sized = not element_bytes or t.itemsize == element_bytes
+    elif t.dtype in types:
+        sized = True
+    elif str(t.dtype) in types.names:
+        types.add(t.dtype)
+        sized = True
+    else:
+        raise MoEError(f"{name}: {' or '.join(types.names)} is needed, got {t.dtype}")
+    if element_bytes and not (sized and t.nbytes >= count * element_bytes and t.is_contiguous()):
         raise MoEError(f"{name}: {count} contiguous values of {element_bytes} bytes are needed, got "
                        f"{tuple(t.shape)} of {t.itemsize} bytes")
     return t.data_ptr()
@@ -261,7 +288,7 @@ def _norm_of(cfg: ResidualNormCfg):
 def _norm_gate(dev: int, name: str, t, cfg: ResidualNormCfg, y_rows) -> Optional[int]:
     if cfg.gate == GATE_ELEMENT:
         return _rows(dev, name, t, y_rows)
-    return _dev(dev, name, t, 4, cfg.tokens if cfg.gate == GATE_TOKEN else cfg.hidden)
+    return _dev(dev, name, t, 4, cfg.tokens if cfg.gate == GATE_TOKEN else cfg.hidden, _F32)
 
 
 class Engine:
@@ -405,7 +432,10 @@ class Engine:
 
     # -- operators around the experts' products ----------------------------
     # Device tensors (contiguous rows, or the row strides of the config); the
-    # tensors' element types are checked against the config's.
+    # tensors' element types are checked against the config's: fp32 weights,
+    # roots and gates, int32 ids and positions, int32 or uint32 indexes, uint8
+    # codes, zero points and E8M0 scales (or torch's own 4- and 8-bit types of
+    # the same bits).
     @staticmethod
     def sort_workspace_bytes(tokens: int, top_k: int, experts: int) -> int:
         return int(load().moe_b200_sort_workspace_bytes(tokens, top_k, experts))
@@ -415,10 +445,11 @@ class Engine:
         """Tokens sorted by expert on the device; int32 tensors, `batches` [min(experts, tokens * top_k), 4]."""
         dev, n = self.device, tokens * top_k
         self._check(self.lib.moe_b200_sort_tokens(
-            self.h, _dev(dev, "ids", ids, 4, n), tokens, top_k, experts, _dev(dev, "position", position, 4, n),
-            _dev(dev, "perm", perm, 4, n), _dev(dev, "offset", offset, 4, experts + 1),
-            _dev(dev, "batches", batches, 4, 4 * min(experts, n)), _dev(dev, "batch_count", batch_count, 4, 1),
-            *_workspace(dev, workspace), stream, self.err))
+            self.h, _dev(dev, "ids", ids, 4, n, _I32), tokens, top_k, experts,
+            _dev(dev, "position", position, 4, n, _I32), _dev(dev, "perm", perm, 4, n, _U32),
+            _dev(dev, "offset", offset, 4, experts + 1, _U32),
+            _dev(dev, "batches", batches, 4, 4 * min(experts, n), _U32),
+            _dev(dev, "batch_count", batch_count, 4, 1, _U32), *_workspace(dev, workspace), stream, self.err))
 
     @staticmethod
     def rows_cfg(hidden: int, tokens: int, top_k: int, sorted_rows: int, token_type: int = DTYPE_BF16,
@@ -428,28 +459,28 @@ class Engine:
     def dispatch_rows(self, cfg: RowsCfg, x, position, sorted, stream: int = 0):
         dev, (t, s, n) = self.device, _rows_of(cfg)
         self._check(self.lib.moe_b200_dispatch_rows(
-            self.h, cfg, _rows(dev, "x", x, t), _dev(dev, "position", position, 4, n),
+            self.h, cfg, _rows(dev, "x", x, t), _dev(dev, "position", position, 4, n, _I32),
             _rows(dev, "sorted", sorted, s), stream, self.err))
 
     def dispatch_rows_backward(self, cfg: RowsCfg, d_sorted, position, d_x, stream: int = 0):
         dev, (t, s, n) = self.device, _rows_of(cfg)
         self._check(self.lib.moe_b200_dispatch_rows_backward(
-            self.h, cfg, _rows(dev, "d_sorted", d_sorted, s), _dev(dev, "position", position, 4, n),
+            self.h, cfg, _rows(dev, "d_sorted", d_sorted, s), _dev(dev, "position", position, 4, n, _I32),
             _rows(dev, "d_x", d_x, t), stream, self.err))
 
     def combine_rows(self, cfg: RowsCfg, sorted, position, w, y, shared=None, stream: int = 0):
         dev, (t, s, n) = self.device, _rows_of(cfg)
         self._check(self.lib.moe_b200_combine_rows(
-            self.h, cfg, _rows(dev, "sorted", sorted, s), _dev(dev, "position", position, 4, n),
-            _dev(dev, "w", w, 4, n), _rows(dev, "shared", shared, t), _rows(dev, "y", y, t), stream, self.err))
+            self.h, cfg, _rows(dev, "sorted", sorted, s), _dev(dev, "position", position, 4, n, _I32),
+            _dev(dev, "w", w, 4, n, _F32), _rows(dev, "shared", shared, t), _rows(dev, "y", y, t), stream, self.err))
 
     def combine_rows_backward(self, cfg: RowsCfg, d_y, sorted, position, w, d_sorted=None, d_w=None,
                               stream: int = 0):
         dev, (t, s, n) = self.device, _rows_of(cfg)
         self._check(self.lib.moe_b200_combine_rows_backward(
             self.h, cfg, _rows(dev, "d_y", d_y, t), _rows(dev, "sorted", sorted, s),
-            _dev(dev, "position", position, 4, n), _dev(dev, "w", w, 4, n), _rows(dev, "d_sorted", d_sorted, s),
-            _dev(dev, "d_w", d_w, 4, n), stream, self.err))
+            _dev(dev, "position", position, 4, n, _I32), _dev(dev, "w", w, 4, n, _F32),
+            _rows(dev, "d_sorted", d_sorted, s), _dev(dev, "d_w", d_w, 4, n, _F32), stream, self.err))
 
     @staticmethod
     def residual_norm_cfg(hidden: int, tokens: int, hidden_type: int = DTYPE_F32, y_type: int = DTYPE_F32,
@@ -465,10 +496,10 @@ class Engine:
                       x=None, rms_y=None, rms_x=None, stream: int = 0):
         dev, (h, b, n, H, T) = self.device, _norm_of(cfg)
         self._check(self.lib.moe_b200_residual_norm_forward(
-            self.h, cfg, _rows(dev, "hidden", hidden, h), _rows(dev, "y", y, b), _dev(dev, "post_w", post_w, 4, H),
-            _norm_gate(dev, "gate", gate, cfg, b), _dev(dev, "pre_w", pre_w, 4, H),
-            _rows(dev, "hidden_out", hidden_out, h), _rows(dev, "x", x, n), _dev(dev, "rms_y", rms_y, 4, T),
-            _dev(dev, "rms_x", rms_x, 4, T), stream, self.err))
+            self.h, cfg, _rows(dev, "hidden", hidden, h), _rows(dev, "y", y, b),
+            _dev(dev, "post_w", post_w, 4, H, _F32), _norm_gate(dev, "gate", gate, cfg, b),
+            _dev(dev, "pre_w", pre_w, 4, H, _F32), _rows(dev, "hidden_out", hidden_out, h), _rows(dev, "x", x, n),
+            _dev(dev, "rms_y", rms_y, 4, T, _F32), _dev(dev, "rms_x", rms_x, 4, T, _F32), stream, self.err))
 
     @staticmethod
     def residual_norm_workspace_bytes(cfg: ResidualNormCfg) -> int:
@@ -480,12 +511,12 @@ class Engine:
         dev, (h, b, n, H, T) = self.device, _norm_of(cfg)
         self._check(self.lib.moe_b200_residual_norm_backward(
             self.h, cfg, _rows(dev, "d_hidden_out", d_hidden_out, h), _rows(dev, "d_x", d_x, n),
-            _rows(dev, "hidden_out", hidden_out, h), _rows(dev, "y", y, b), _dev(dev, "post_w", post_w, 4, H),
-            _norm_gate(dev, "gate", gate, cfg, b), _dev(dev, "pre_w", pre_w, 4, H), _dev(dev, "rms_y", rms_y, 4, T),
-            _dev(dev, "rms_x", rms_x, 4, T), _rows(dev, "d_hidden", d_hidden, h), _rows(dev, "d_y", d_y, b),
-            _dev(dev, "d_post_w", d_post_w, 4, H), _norm_gate(dev, "d_gate", d_gate, cfg, b),
-            _dev(dev, "d_pre_w", d_pre_w, 4, H),
-            *_workspace(dev, workspace), stream, self.err))
+            _rows(dev, "hidden_out", hidden_out, h), _rows(dev, "y", y, b), _dev(dev, "post_w", post_w, 4, H, _F32),
+            _norm_gate(dev, "gate", gate, cfg, b), _dev(dev, "pre_w", pre_w, 4, H, _F32),
+            _dev(dev, "rms_y", rms_y, 4, T, _F32), _dev(dev, "rms_x", rms_x, 4, T, _F32),
+            _rows(dev, "d_hidden", d_hidden, h), _rows(dev, "d_y", d_y, b),
+            _dev(dev, "d_post_w", d_post_w, 4, H, _F32), _norm_gate(dev, "d_gate", d_gate, cfg, b),
+            _dev(dev, "d_pre_w", d_pre_w, 4, H, _F32), *_workspace(dev, workspace), stream, self.err))
 
     @staticmethod
     def q4_cfg(rows: int, cols: int, tokens: int, out_rows: int = 0, code: int = Q4_E2M1, group: int = 32,
@@ -501,12 +532,12 @@ class Engine:
         groups = rows * cfg.cols // cfg.group if cfg.group else 0
         dev, out = self.device, cfg.out_rows or cfg.tokens
         self._check(self.lib.moe_b200_q4_matvec(
-            self.h, cfg, _dev(dev, "codes", codes, 1, rows * cfg.cols // 2),
-            _dev(dev, "scales", scales, _TYPE_BYTES.get(cfg.scale_type, 0), groups),
-            _dev(dev, "zeros", zeros, 1, groups),
+            self.h, cfg, _dev(dev, "codes", codes, 1, rows * cfg.cols // 2, _CODES.get(cfg.code)),
+            _dev(dev, "scales", scales, _TYPE_BYTES.get(cfg.scale_type, 0), groups, _SCALES.get(cfg.scale_type)),
+            _dev(dev, "zeros", zeros, 1, groups, _U8),
             _rows(dev, "x", x, (cfg.x_type, cfg.tokens, cfg.cols, cfg.x_stride)),
-            _dev(dev, "batches", batches, 4, 4 * min(cfg.experts or 1, out)),
-            _dev(dev, "batch_count", batch_count, 4, 1), _dev(dev, "perm", perm, 4, out),
+            _dev(dev, "batches", batches, 4, 4 * min(cfg.experts or 1, out), _U32),
+            _dev(dev, "batch_count", batch_count, 4, 1, _U32), _dev(dev, "perm", perm, 4, out, _U32),
             _rows(dev, "y", y, (cfg.y_type, out, cfg.rows, cfg.y_stride)), stream, self.err))
 
     # -- expert parallelism ------------------------------------------------
