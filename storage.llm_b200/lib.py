@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import re
+import threading
 from pathlib import Path
 from typing import Optional
 
@@ -297,11 +298,20 @@ class Engine:
     def __init__(self, device: int = 0, max_layers: int = 1):
         self.lib = load()
         self.device = device
-        self.err = C.create_string_buffer(ERR_LEN)
+        self._errs = threading.local()
         init = InitT(device, max_layers)
         self.h = self.lib.moe_b200_create(C.byref(init), self.err)
         if not self.h:
             raise MoEError(self.err.value.decode())
+
+    @property
+    def err(self):
+        """The calling thread's error buffer: calls of other threads run during one of its own."""
+        try:
+            return self._errs.buf
+        except AttributeError:
+            self._errs.buf = C.create_string_buffer(ERR_LEN)
+            return self._errs.buf
 
     def _check(self, ok: int):
         if not ok:

@@ -3,6 +3,7 @@ configs that no call takes, tensors of another element type, calls from two
 threads.  Without a GPU, like test_operators_cpu.py."""
 import subprocess
 import sys
+import threading
 from pathlib import Path
 
 import pytest
@@ -21,6 +22,7 @@ def L(pkg):
 
 QUERY = """
 import sys
+import threading
 sys.path.insert(0, sys.argv[1])
 import conftest
 conftest.load_pkg()
@@ -150,3 +152,28 @@ def test_types_with_the_same_meaning_are_taken(L, face):
     eng.sort_tokens(t((8,), I32), 4, 2, 8, position=t((8,), I32), perm=t((8,), U32), offset=t((9,), U32),
                     batches=t((8, 4), U32), batch_count=t((1,), U32))
     assert len(lib.calls) == 7
+
+
+def test_refusals_of_two_threads_keep_their_messages(L, face):
+    """Two calls of one engine refused at once: neither returns before both have
+    written their messages, and each thread's error is its own."""
+    both = threading.Barrier(2, timeout=30)
+
+    def refuse(engine, stream, err):
+        err.value = b"stream %d" % stream
+        both.wait()
+        return 0
+    eng, _ = face(moe_b200_sync=refuse)
+    said = {}
+
+    def work(stream):
+        try:
+            eng.sync(stream)
+        except L.MoEError as e:
+            said[stream] = str(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in (1, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert said == {1: "stream 1", 2: "stream 2"}
