@@ -518,8 +518,8 @@ typedef struct {
     int32_t gate_sigmoid;
     int32_t norm_unit_offset; /* the norms multiply by (1 + w) */
     float norm_eps;           /* <= 0 -> 1e-6 */
-    float residual_scale;     /* 0 -> 1 */
-    float out_scale;          /* 0 -> 1 */
+    float residual_scale;     /* 0 -> 1, also where a caller's own scale reaches 0 */
+    float out_scale;          /* 0 -> 1, likewise: leave y NULL for a branch that counts nothing */
     uint64_t hidden_stride;   /* row strides; a gradient's rows have its tensor's */
     uint64_t y_stride;
     uint64_t x_stride;

@@ -498,9 +498,15 @@ class Engine:
                           norm_unit_offset: bool = False, norm_eps: float = 0.0, residual_scale: float = 1.0,
                           out_scale: float = 1.0, hidden_stride: int = 0, y_stride: int = 0,
                           x_stride: int = 0) -> ResidualNormCfg:
-        return ResidualNormCfg(hidden, tokens, hidden_type, y_type, x_type, gate, int(gate_sigmoid),
-                               int(norm_unit_offset), norm_eps, residual_scale, out_scale, hidden_stride, y_stride,
-                               x_stride)
+        """A scale of 0 is refused: in the C config it stands for one that is not set, which is 1."""
+        cfg = ResidualNormCfg(hidden, tokens, hidden_type, y_type, x_type, gate, int(gate_sigmoid),
+                              int(norm_unit_offset), norm_eps, residual_scale, out_scale, hidden_stride, y_stride,
+                              x_stride)
+        for name, given in (("residual_scale", residual_scale), ("out_scale", out_scale)):
+            if getattr(cfg, name) == 0.0:  # as fp32
+                raise MoEError(f"{name}={given} is 0 in fp32, which stands for 1; call without y to leave the "
+                               "block's output out")
+        return cfg
 
     def residual_norm(self, cfg: ResidualNormCfg, hidden, y=None, post_w=None, gate=None, pre_w=None, hidden_out=None,
                       x=None, rms_y=None, rms_x=None, stream: int = 0):

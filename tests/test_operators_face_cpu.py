@@ -177,3 +177,13 @@ def test_refusals_of_two_threads_keep_their_messages(L, face):
     for t in threads:
         t.join()
     assert said == {1: "stream 1", 2: "stream 2"}
+
+
+@pytest.mark.parametrize("name", ["residual_scale", "out_scale"])
+def test_scales_of_zero_are_refused(L, name):
+    """A zero (or what becomes one in fp32) would stand for 1 in the C config."""
+    for value in (0.0, -0.0, 1e-50):
+        with pytest.raises(L.MoEError, match=name):
+            L.Engine.residual_norm_cfg(64, 4, **{name: value})
+    for value in (1.0, -0.5, 1e-40):
+        assert getattr(L.Engine.residual_norm_cfg(64, 4, **{name: value}), name) != 0.0
