@@ -546,7 +546,11 @@ class Engine:
                   stream: int = 0):
         rows = (cfg.experts or 1) * cfg.rows * (2 if cfg.gated else 1)
         groups = rows * cfg.cols // cfg.group if cfg.group else 0
-        dev, out = self.device, cfg.out_rows or cfg.tokens
+        dev, out = self.device, cfg.out_rows
+        if batches is None:
+            out = out or cfg.tokens
+        elif out == 0 and y is not None and y.shape[0]:
+            raise MoEError(f"out_rows=0 with batches and a y of {y.shape[0]} rows, none of which would be written")
         self._check(self.lib.moe_b200_q4_matvec(
             self.h, cfg, _dev(dev, "codes", codes, 1, rows * cfg.cols // 2, _CODES.get(cfg.code)),
             _dev(dev, "scales", scales, _TYPE_BYTES.get(cfg.scale_type, 0), groups, _SCALES.get(cfg.scale_type)),

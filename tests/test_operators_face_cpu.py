@@ -187,3 +187,22 @@ def test_scales_of_zero_are_refused(L, name):
             L.Engine.residual_norm_cfg(64, 4, **{name: value})
     for value in (1.0, -0.5, 1e-40):
         assert getattr(L.Engine.residual_norm_cfg(64, 4, **{name: value}), name) != 0.0
+
+
+def test_products_by_expert_take_out_rows_as_it_is(L, face):
+    """A rank to which no row was routed has an empty y, whatever the tokens; a
+    config without out_rows for a y that has rows would leave them unwritten."""
+    eng, lib = face()
+    by = dict(batches=tensor((8, 4), I32), batch_count=tensor((1,), I32), perm=tensor((32,), I32))
+    args = tensor((8, 48, 32), U8), tensor((8, 48, 2), U8), tensor((16, 64), BF16)
+    cfg = L.Engine.q4_cfg(48, 64, 16, 0, experts=8, top_k=2)
+    eng.q4_matvec(cfg, *args, tensor((0, 48), F32), **by)
+    assert len(lib.calls) == 1
+    with pytest.raises(L.MoEError, match="out_rows=0 .* y of 32 rows"):
+        eng.q4_matvec(cfg, *args, tensor((32, 48), F32), **by)
+    assert len(lib.calls) == 1
+    eng.q4_matvec(L.Engine.q4_cfg(48, 64, 16, 32, experts=8, top_k=2), *args, tensor((32, 48), F32), **by)
+    # without batches 0 stands for the tokens
+    eng.q4_matvec(L.Engine.q4_cfg(48, 64, 16), tensor((48, 32), U8), tensor((48, 2), U8), args[2],
+                  tensor((16, 48), F32))
+    assert len(lib.calls) == 3
