@@ -204,6 +204,13 @@ class MoEError(RuntimeError):
     pass
 
 
+class _ErrorBuffer(threading.local):
+    """`buf`: one a thread, made when the thread first asks."""
+
+    def __init__(self):
+        self.buf = C.create_string_buffer(ERR_LEN)
+
+
 _TYPE_BYTES = {DTYPE_F32: 4, DTYPE_BF16: 2, DTYPE_F16: 2, DTYPE_E8M0: 1}
 _KIND = {}  # torch dtype -> DTYPE_*, filled as types are met (this module does not import torch)
 
@@ -234,15 +241,13 @@ def _dev(dev: int, name: str, t, element_bytes: int, count: int, types: Optional
     if t.get_device() != dev:
         raise MoEError(f"{name} is on {t.device}, the engine on cuda:{dev}")
     if types is None:
-        sized = not element_bytes or t.itemsize == element_bytes
-    elif t.dtype in types:
-        sized = True
-    elif str(t.dtype) in types.names:
+        if element_bytes and t.itemsize != element_bytes:
+            raise MoEError(f"{name}: values of {element_bytes} bytes are needed, got {t.dtype}")
+    elif t.dtype not in types:
+        if str(t.dtype) not in types.names:
+            raise MoEError(f"{name}: {' or '.join(types.names)} is needed, got {t.dtype}")
         types.add(t.dtype)
-        sized = True
-    else:
-        raise MoEError(f"{name}: {' or '.join(types.names)} is needed, got {t.dtype}")
-    if element_bytes and not (sized and t.nbytes >= count * element_bytes and t.is_contiguous()):
+    if element_bytes and (t.nbytes < count * element_bytes or not t.is_contiguous()):
         raise MoEError(f"{name}: {count} contiguous values of {element_bytes} bytes are needed, got "
                        f"{tuple(t.shape)} of {t.itemsize} bytes")
     return t.data_ptr()
@@ -298,7 +303,7 @@ class Engine:
     def __init__(self, device: int = 0, max_layers: int = 1):
         self.lib = load()
         self.device = device
-        self._errs = threading.local()
+        self._errs = _ErrorBuffer()
         init = InitT(device, max_layers)
         self.h = self.lib.moe_b200_create(C.byref(init), self.err)
         if not self.h:
@@ -307,11 +312,7 @@ class Engine:
     @property
     def err(self):
         """The calling thread's error buffer: calls of other threads run during one of its own."""
-        try:
-            return self._errs.buf
-        except AttributeError:
-            self._errs.buf = C.create_string_buffer(ERR_LEN)
-            return self._errs.buf
+        return self._errs.buf
 
     def _check(self, ok: int):
         if not ok:
