@@ -419,8 +419,9 @@ MOE_B200_API int moe_b200_ep_last_counts(moe_b200_engine_t* engine, uint32_t* se
  *     buffer that no result belongs to are left as they were.
  * Row strides are in elements, 0 = rows back to back.  Outputs must not
  * overlap inputs or each other, but for the pairs named below.  The fast
- * kernels need 16-byte aligned rows (pointer and stride); other rows run
- * element by element.
+ * row and norm kernels need rows of a multiple of 8 columns on 16-byte
+ * boundaries (pointer and stride); other rows run element by element, and their
+ * sums, added in another order, differ in the last places.
  * ------------------------------------------------------------------------ */
 enum {
     MOE_B200_DTYPE_F32 = 0,
@@ -552,8 +553,10 @@ MOE_B200_API int moe_b200_residual_norm_backward(moe_b200_engine_t* engine, cons
 
 /* Matrix-vector products with 4-bit weights and group scales, for single
  * tokens and small batches: y[r, n] = sum_g scale[n, g] * sum_{k in g}
- * value(code[n, k]) * x[r, k], products exact, sums in fp32.  Plain layouts,
- * nothing repacked:
+ * value(code[n, k]) * x[r, k], products exact, sums in fp32 (of 2^-16 of the
+ * values, so that a group's sum does not overflow before its scale: x below
+ * 2^-86 in fp32 or 2^-109 in bf16 may lose bits below fp32's normal numbers).
+ * Plain layouts, nothing repacked:
  *   codes    [experts][rows][cols / 2], column 2i in the low nibble of byte i
  *   scales   [experts][rows][cols / group] of scale_type
  *   zeros    [experts][rows][cols / group] uint8 zero points of integer codes

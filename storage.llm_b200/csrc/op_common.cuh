@@ -153,7 +153,9 @@ __device__ __forceinline__ void load_f32(const float* p, float* v) {
 
 // ---------------------------------------------------------------------------
 // Vectors of V fp32 values; for V = 4 and 8 two values an instruction.  Nothing is
-// contracted, so every kernel that forms a value gives the same bits.
+// contracted, so the general and the specialised kernels of one V give the same
+// bits.  Kernels of another V give threads other columns and vdot other sums:
+// their sums over a row differ in the last places.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ uint64_t two(float lo, float hi) {
     uint64_t v;

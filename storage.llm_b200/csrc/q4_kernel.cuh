@@ -29,14 +29,19 @@
 //     multiply-add brings either into range and takes the zero point off.
 // Measured, with the share of a copy's 6.55 TB/s and what bounds it:
 //   131,072 x 7168 integers by 128, 4 rows           110 us, 69 %   instructions
-//   64 rows of 256 gated MXFP4 experts 2 x 2048 x 7168   225 us, 61 %   instructions:
-//       17 decode 8 codes; on 131,072 x 7168 one row's 99 million are 90 us at
-//       full issue, 134 us as measured
+//   64 rows of 256 gated MXFP4 experts 2 x 2048 x 7168   225 us, 61 %   instructions and
+//       their latency: 17 decode 8 codes; on 131,072 x 7168 one row's 99 million
+//       are 90 us at full issue, 134 us as measured, with 16 warps an SM
 //   128 fp32 rows of 32 MXFP4 experts 2880 x 2880     75 us, 29 %   instructions: the three
 //       terms cost a third of a slice's; blocks of 9 to 16 rows go twice
 //   7168 x 2048 MXFP4, one row                         5.1 us        launch and latency
 //   131,072 x 7168 integers, 32 rows                 337 us, 22 %   latency: four tiles of
 //       sums leave registers for 8 warps an SM
+//   rows of x off 16-byte boundaries (staged in shared memory, one launch shape):
+//       7168 x 2048 one row 6.3 us for 5.3, 131,072 x 7168 one row 180 for 135,
+//       16,384 x 4096 8 bf16 rows 48 for 15, 4 fp32 rows 119 for 20
+//   few outputs: 256 x 8192, one row 6.3 us on 16 SMs; 32 fp32 rows 46 us, four
+//       passes one after the other on 8
 // Slower, each by its measured time: blocks that stay for several tiles (their
 // beginnings and ends no longer cover each other), warps with rows of their own
 // and all columns (32 rows: 380 us), 128 registers for four tiles (479 us).

@@ -374,12 +374,24 @@ __device__ __forceinline__ void store_own(float* row, uint32_t c, uint32_t H, co
 // is the gate's kind (a token's or none: 0), otherwise -1.
 // 4,096 x 2048 bf16 with an element gate: 35.2 us, 58 % (87 us when the loads
 // waited for each row and neighbouring threads' sums met the same banks).
-// What bounds it: instructions (some 640 for a warp's 256 columns, a third of
-// them a row's own, whatever it holds; issued in 62 % of the cycles) and the
-// sums over the tokens in shared memory.  A thread to 16 columns would halve
-// the rows' own instructions but holds 4 blocks of 128 threads an SM: 61 us.
+// What bounds it: too little overlap for what each row costs.  A warp issues some
+// 640 instructions for its 256 columns, a third of them the row's own, and reads
+// and writes every sum over the tokens in shared memory; with 36 % of an SM's
+// warps resident and a barrier every row, issue is busy in 59 % of the cycles
+// and the path to shared memory in 64 %.  A thread to 16 columns would halve the
+// rows' own instructions but leaves 4 blocks of 128 threads an SM: 61 us.
+// Above 4096 columns one block of up to 1024 threads, spilling some of its 64
+// registers, holds an SM, and beside the sums its ring often has one place, so
+// that copies wait for the row before: 4,096 x 7168 with an fp32 stream, bf16
+// rows and a channel gate 214 us (38 %), 8192 columns bf16 181 us (34 %).  Above
+// 8192 (N = 0): 2,048 x 12,288 bf16 192 us (24 %), 16,384 columns 267 us.
 // Rows that cannot be read by vectors take one column an instruction: 4,096 x
-// 2043 62 us (25 %), 2,048 x 5001 142 us, 192 with branches around its loads.
+// 2043 62 us (25 %), 2,048 x 5001 140 us, 192 with branches around its loads.
+// GATE >= 0 against the general kernel (us; none, channel and element gate, bf16,
+// through a sigmoid): 4,096 x 2048 26 41 35 and 38 48 47; 4,096 x 4096 44 62 52
+// and 52 71 67; 4,096 x 7168 97 149 and 144 183; 4,096 x 2043 55 74 73 and 95 124
+// 116; 2,048 x 5001 103 140 and 220 249.  Element gates above 4096 columns
+// run by the general kernel: 4,096 x 7168 173 us, 2,048 x 5001 266.
 template <typename DH, typename DY, typename DX, int V, int N, bool BULK, int GATE, uint32_t THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
     norm_backward_kernel(const typename DH::type* d_hidden_out, const typename DX::type* d_x,
@@ -768,7 +780,7 @@ cudaError_t run_forward(const NormArgs& a, const NormJob& job, bool vec, const S
         return full ? go(norm_forward_kernel<DH, DY, DX, 4, 4, true, R, 128, 8>, nullptr, 0, warps, few)
                     : go(norm_forward_kernel<DH, DY, DX, 4, 4, false, R, 128, 8>, nullptr, 0, warps, few);
     }
-    // 16 columns a thread
+    // 16 columns a thread; 8 where they are read one by one, up to 4096 of them
     if (const uint32_t n = vec ? 0 : row_threads(job.H, 8, 512)) {
         return full ? go(norm_forward_kernel<DH, DY, DX, 1, 8, true, 1, 512, 2>, nullptr, 0, n, job.T)
                     : go(norm_forward_kernel<DH, DY, DX, 1, 8, false, 1, 512, 2>, nullptr, 0, n, job.T);
